@@ -15,9 +15,9 @@
 //  * the survivor bit of a step ("odd predecessor wins", lane order of time t+1) is shifted into a per-lane
 //    accumulator (v_cmp -> vcc -> v_addc_co_u32 acc, acc, acc); every C8P_SV_BLK = 30 steps the wave stores its 64
 //    accumulators with one coalesced 256-byte vector store.  Block b of a packet = 64 dwords, dword[lane] bit
-//    (29 - k) = decision of step 30 b + k.  (The first version stored the ballot word of every step through
-//    s_store_dwordx4: the scalar store path capped the kernel at 0.80 ms per 4096 packets against 0.47-0.57 ms
-//    without stores; the accumulate costs one more VALU instruction per step and no scalar-memory traffic.)
+//    (29 - k) = decision of step 30 b + k.  (The first version stored the ballot word of every step from SGPRs, and
+//    that path capped the kernel at 0.80 ms per 4096 packets against 0.47-0.57 ms without stores; the accumulate costs
+//    one more VALU instruction per step and no scalar-memory traffic.)
 //
 // Exactness.  The kernel drops the reference's -1e15 clamp and its "neither candidate beat the pre-fill" record.
 // For LLRs that are all finite with |LLR| <= 2^20 this is the identical function (DESIGN.md "lean = exact"):
