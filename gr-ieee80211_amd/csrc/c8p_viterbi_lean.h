@@ -55,7 +55,7 @@ template <int Q> __device__ __forceinline__ unsigned long long lane_bit_mask()
 // DPP operands sit inside inline asm, invisible to the compiler's hazard recogniser: a VGPR written by VALU needs
 // 2 wait states before a DPP read, hence the leading "s_nop 1" of every DPP block.
 typedef float v2f __attribute__((ext_vector_type(2)));
-struct LeanK {          // lane constants for one exchange phase q, as the register pairs the packed instructions read
+struct LeanK {          // lane constants for one exchange phase q
   v2f a;                // {ka, sa}: keep / send coefficient of t0   tab[c] = ka*t0 + kb*t1, tab[3-c] = sa*t0 + sb*t1
   v2f b;                // {kb, sb}: keep / send coefficient of t1
   int cls;              // v_cmp_class mask for d = recv - keep (q <= 3)
@@ -64,8 +64,8 @@ struct LeanK {          // lane constants for one exchange phase q, as the regis
 #define C8P_CLS_POS 0x380   // +denormal | +normal | +inf
 #define C8P_CLS_NEG 0x01C   // -inf | -normal | -denormal
 
-// keep and send are the same arithmetic on (ka,kb) and (sa,sb): one packed-f32 instruction does both
-// (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32 are two independent IEEE operations, no cross-element effects).
+// keep and send are the same arithmetic on (ka,kb) and (sa,sb): two independent IEEE operations, one plain instruction each
+// (no packed FP32: the Makefile switches it off).
 template <bool HAVE0, bool HAVE1>
 __device__ __forceinline__ v2f cand2(float pre, const LeanK& k, float t0, float t1)
 {

@@ -1,9 +1,17 @@
 """What no GPU source of this tree may hold, checked on its text (CPU only: no GPU, no build).
 
 Scalar data cache: GPU code here never WRITES through it (scalar stores, scalar atomics, that cache's write-back and discard).  The
-survivors, the one place that ever did, leave through coalesced vector stores."""
+survivors, the one place that ever did, leave through coalesced vector stores.
+
+Packed FP32: no instruction that works on a register pair of floats, written by hand or formed by the compiler (some of their forms have
+given wrong results on this hardware, now and then and without an error): the text of the sources, every line that calls hipcc, and the
+assembly of the library's two builds (cross-compiled here with the Makefile's own command lines)."""
 import os
 import re
+import shlex
+import subprocess
+
+import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 SKIP = {".git", "__pycache__", ".pytest_cache", "gpurun_out", "_work", "build", "profiles", "node_modules"}
@@ -48,3 +56,55 @@ def test_pattern_knows_the_instructions():
 
 def test_no_source_writes_through_the_scalar_data_cache():
     assert hits(SCALAR_CACHE_WRITE) == []
+
+
+PACKED_FP32 = re.compile(r"\bv_pk_(?:add|mul|fma)_" + "f32")
+
+
+def test_no_source_holds_a_packed_fp32_instruction():
+    assert hits(PACKED_FP32) == []
+
+
+def test_every_hipcc_line_switches_packed_fp32_off():
+    """a file that gives hipcc its --offload-arch gives it the feature switch too, as often"""
+    seen, bad = [], []
+    arch, off = re.compile(r"--offload-arch="), re.compile(r"-Xclang -target-feature -Xclang -packed-fp32-ops")
+    for p in source_files():
+        if os.path.abspath(p) == os.path.abspath(__file__):
+            continue
+        text = open(p, errors="replace").read()
+        n = len([m for m in arch.finditer(text)])
+        if n:
+            seen.append(os.path.relpath(p, ROOT))
+            if len(off.findall(text)) != n:
+                bad.append(os.path.relpath(p, ROOT))
+    assert {"gr-ieee80211_amd/csrc/Makefile", "gnuradio/CMakeLists.txt", "tools/hipflags.sh"} <= set(seen)
+    assert bad == []
+
+
+@pytest.fixture(scope="module")
+def assembly(tmp_path_factory):
+    """{library: device assembly}, built with the command lines that make would run for the libraries"""
+    csrc = os.path.join(ROOT, "gr-ieee80211_amd", "csrc")
+    tmp, running, out = tmp_path_factory.mktemp("asm"), {}, {}
+    for lib in ("../libc8p_rx.so", "../libc8p_rx_exp.so"):
+        line = subprocess.run(["make", "-s", "-n", "-B", "-C", csrc, lib], capture_output=True, text=True, timeout=60)
+        assert line.returncode == 0, line.stderr
+        cmd = shlex.split(line.stdout.strip().splitlines()[-1])
+        assert cmd[cmd.index("-o") + 1] == lib and "-shared" in cmd, cmd
+        dst = str(tmp / (os.path.basename(lib) + ".s"))
+        cmd[cmd.index("-o") + 1] = dst
+        cmd[cmd.index("-shared")] = "-S"
+        running[lib] = (subprocess.Popen(cmd + ["--cuda-device-only"], cwd=csrc, stdout=subprocess.DEVNULL, stderr=subprocess.PIPE, text=True), dst)
+    for lib, (p, dst) in running.items():
+        err = p.communicate(timeout=900)[1]
+        assert p.returncode == 0, err[-2000:]
+        out[lib] = open(dst).read()
+    return out
+
+
+def test_the_built_kernels_hold_no_packed_fp32_and_no_scalar_cache_write(assembly):
+    for lib, text in assembly.items():
+        assert "k_rx_1ss_lds" in text and "v_fma_f32" in text, lib
+        assert PACKED_FP32.search(text) is None, (lib, PACKED_FP32.search(text).group(0))
+        assert SCALAR_CACHE_WRITE.search(text) is None, (lib, SCALAR_CACHE_WRITE.search(text).group(0))

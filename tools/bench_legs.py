@@ -496,15 +496,15 @@ def sensitivity_legs(torch, dev, local, n_pkt, headline, window_s=0.12, deadline
 
 def lean_step_mix(T, float_frac=0.0, cr_num=5):
     """VALU wave-instructions of the lean forward pass per packet of T trellis steps at code rate 5/6, by opcode, from the kernel's
-    structure (csrc/c8p_viterbi_lean.h, tools/gen_lean_asm.py): every step one packed candidate fma, steps with both LLRs present
-    (1 in 5) a packed mul + add more.  Integer-compare blocks (path metrics provably positive): exchange phases q=0,1,3 a borrow
+    structure (csrc/c8p_viterbi_lean.h, tools/gen_lean_asm.py): every step two candidates, one fma each, or with both LLRs present
+    (1 step in 5) one mul, one fmac and one add each.  Integer-compare blocks (path metrics provably positive): exchange phases q=0,1,3 a borrow
     (v_subb_co_u32_dpp) and v_max_u32_dpp, q=2 one mov_dpp more, q=4,5 permlane swap + v_max_u32 + v_sub_co_u32; one carry-shift per
-    step: 147 per 30 steps.  Float blocks (the fraction `float_frac`, measured in this run): sub_dpp + max_dpp + class test: 167."""
+    step: 189 per 30 steps.  Float blocks (the fraction `float_frac`, measured in this run): sub_dpp + max_dpp + class test: 209."""
     assert cr_num == 5
-    per30_int = {"v_pk_fma_f32": 30, "v_pk_mul_f32": 6, "v_pk_add_f32": 6, "v_subb_co_u32_dpp": 20, "v_max_u32_dpp": 20,
+    per30_int = {"v_fma_f32": 48, "v_mul_f32": 12, "v_fmac_f32": 12, "v_add_f32": 12, "v_subb_co_u32_dpp": 20, "v_max_u32_dpp": 20,
                  "v_mov_b32_dpp": 5, "v_permlane16_swap_b32": 5, "v_permlane32_swap_b32": 5, "v_max_u32": 10,
                  "v_sub_co_u32": 10, "v_addc_co_u32": 30, "v_xor_b32": 1}
-    per30_flt = {"v_pk_fma_f32": 30, "v_pk_mul_f32": 6, "v_pk_add_f32": 6, "v_sub_f32_dpp": 20, "v_max_f32_dpp": 20,
+    per30_flt = {"v_fma_f32": 48, "v_mul_f32": 12, "v_fmac_f32": 12, "v_add_f32": 12, "v_sub_f32_dpp": 20, "v_max_f32_dpp": 20,
                  "v_mov_b32_dpp": 5, "v_permlane16_swap_b32": 5, "v_permlane32_swap_b32": 5, "v_max_f32": 10,
                  "v_cmp_class_f32": 20, "v_cmp_gt_f32": 10, "v_addc_co_u32": 30}
     mix = {}
@@ -530,6 +530,8 @@ def valu_roofline(kern_x, n_pkt, float_frac, profile_tag, T=11960):
         return None
     cost = json.load(open(f_cost))["lean_step_opcodes"]
     mix = lean_step_mix(T, float_frac)
+    if any(k not in cost for k in mix):                            # a table taken with another step prices nothing here
+        return None
     dec_instr = sum(mix.values()) * n_pkt
     cycles = sum(mix[k] * cost[k] for k in mix) * n_pkt            # SIMD-cycles summed over the chip
     other, other_src, busy = 0.0, None, None

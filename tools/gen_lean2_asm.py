@@ -11,8 +11,8 @@ step with both LLRs is computed once per wave-step and shared by the two registe
 16 lanes x 4 registers; this is the half-way layout that still gives a 4096-packet batch two waves per SIMD).
 
 What differs per register is a compile-time fact: the class of a transition is GF(2)-linear in D, so register 1 sees class
-c XOR delta(q).  delta = 3 swaps the keep / send halves of the lane-constant coefficient pair (an op_sel), delta = 1 or 2 swaps only
-the t1 or only the t0 coefficient.
+c XOR delta(q).  delta = 3 swaps the keep and send coefficients of the lane, delta = 1 or 2 swaps only those of t1 or only those of t0
+(another operand in the text of the instruction, no cost).
 
 LLRs: every lane reads ITS packet's LDS buffer (two addresses per instruction, a broadcast inside each half of the wave) with
 ds_read_b64 into rotating register pairs, scheduled exactly as in lean_blocks_lds (tools/gen_lean_asm.py, gen_rate_lds): the read of
@@ -31,6 +31,7 @@ import sys
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 from gen_lean4_asm import idx, keep_class          # noqa: E402  (the same puncture patterns and transition classes)
+from gen_lean_asm import coeffs                    # noqa: E402
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 OUT = os.environ.get("C8P_GEN_OUT2") or os.path.join(ROOT, "gr-ieee80211_amd", "csrc", "c8p_lean2_asm.h")
@@ -71,9 +72,8 @@ def gen_rate(cr):
     def lreg(i):
         return VB + SW * (grp(i) % NS) + (i % GS)
 
-    def lpair(i):
-        r = lreg(i)
-        return "v[%d:%d]" % (r & ~1, (r & ~1) + 1), r & 1
+    def llr(i):
+        return "v%d" % lreg(i)
 
     def load_group(g, wrapped):
         off = 4 * GS * g + (4 * n if wrapped else 0)
@@ -96,31 +96,33 @@ def gen_rate(cr):
         dl = (0, delta(q))
         # ---- candidates of both registers
         if i0 is not None and i1 is not None:
-            p0, s0 = lpair(i0)
-            p1, s1 = lpair(i1)
             tabs = {}
             for kind in sorted(set(0 if d in (0, 3) else 1 for d in dl)):
                 t = TAB[len(tabs)]
                 tabs[kind] = t
                 # kind 0: {ka t0 + kb t1, sa t0 + sb t1};  kind 1: the t1 coefficients swapped {ka t0 + sb t1, sa t0 + kb t1}
                 sb = 1 if kind == 1 else 0
-                emit("v_pk_mul_f32 v[%d:%d], %%[kb%d], %s op_sel:[%d,%d] op_sel_hi:[%d,%d]" % (t, t + 1, q, p1, sb, s1, 1 - sb, s1), [grp(i1)])
-                emit("v_pk_fma_f32 v[%d:%d], %%[ka%d], %s, v[%d:%d] op_sel:[0,%d,0] op_sel_hi:[1,%d,1]" % (t, t + 1, q, p0, t, t + 1, s0, s0), [grp(i0)])
+                for h in (0, 1):
+                    emit("v_mul_f32_e32 v%d, %s, %%[%sb%d]" % (t + h, llr(i1), "ks"[h ^ sb], q), [grp(i1)])
+                for h in (0, 1):
+                    emit("v_fmac_f32_e32 v%d, %s, %%[%sa%d]" % (t + h, llr(i0), "ks"[h], q), [grp(i0)])
             for r in range(2):
                 d = dl[r]
                 t = tabs[0 if d in (0, 3) else 1]
                 sw = 1 if d in (3, 2) else 0
-                emit("v_pk_add_f32 v[%d:%d], v[%d:%d], v[%d:%d] op_sel:[0,%d] op_sel_hi:[0,%d]" % (C[r], C[r] + 1, M[r], M[r] + 1, t, t + 1, sw, 1 - sw))
+                for h in (0, 1):
+                    emit("v_add_f32_e32 v%d, v%d, v%d" % (C[r] + h, M[r], t + (h ^ sw)))
         else:
             for r in range(2):
                 d = dl[r]
                 if i0 is not None:
-                    (p, s), sw, kk, ii = lpair(i0), (d >> 1) & 1, "ka", i0
+                    sw, k, i = (d >> 1) & 1, "a", i0
                 else:
-                    (p, s), sw, kk, ii = lpair(i1), d & 1, "kb", i1
-                emit("v_pk_fma_f32 v[%d:%d], %%[%s%d], %s, v[%d:%d] op_sel:[%d,%d,0] op_sel_hi:[%d,%d,0]" % (C[r], C[r] + 1, kk, q, p, M[r], M[r] + 1, sw, s, 1 - sw, s), [grp(ii)])
+                    sw, k, i = d & 1, "b", i1
+                for h in (0, 1):
+                    emit("v_fma_f32 v%d, %%[%s%s%d], %s, v%d" % (C[r] + h, "ks"[h ^ sw], k, q, llr(i), M[r]), [grp(i)])
         # ---- exchange, decision, record (a DPP / permlane read needs two wait states after the VALU write of its source: register 1's
-        #      candidates are one instruction away from register 0's exchange)
+        #      send candidate is the last thing written)
         if q in DPP:
             emit("s_nop 0")
             for r in range(2):
@@ -248,7 +250,7 @@ def gen_rate(cr):
     text = "\n".join('      "%s\\n\\t"' % x for x in L)
     fixed = (M[0], M[1], VOFF, LADDR)
     clob = ['"vcc"', '"scc"', '"memory"'] + ['"s%d"' % (PTR + i) for i in range(8)] + ['"v%d"' % r for r in range(VB, 64) if r not in fixed]
-    ins = ['[ka%d] "v"(K[%d].a)' % (q, q) for q in range(6)] + ['[kb%d] "v"(K[%d].b)' % (q, q) for q in range(6)] + \
+    ins = coeffs() + \
           ['[initx] "v"(initx)', '[inity] "v"(inity)', '[flip] "v"(flip)', '[bound] "v"(bound)', '[segn] "s"(segn)', '[sv] "s"(sv)']
     return """
 // code rate %s: %d LLRs per block in %d groups of %d, %d register sets (v%d..v43); %d VALU instructions per 30 wave-steps = %.1f per packet

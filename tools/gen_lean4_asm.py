@@ -10,8 +10,8 @@ is four plain VALU instructions (candidates, max, borrow, record) instead of the
 a step with both LLRs is computed once per wave-step and shared by the four registers.
 
 What differs per register is a compile-time fact: the class of a transition is GF(2)-linear in D, so register r sees class c XOR
-delta(q, r).  delta = 3 swaps the keep / send halves of the lane-constant coefficient pair (an op_sel), delta = 1 or 2 swaps only
-the t1 or only the t0 coefficient.
+delta(q, r).  delta = 3 swaps the keep and send coefficients of the lane, delta = 1 or 2 swaps only those of t1 or only those of t0
+(another operand in the text of the instruction, no cost).
 
 LLRs are per-row values: each lane reads its packet's stream with 16-byte vector loads (the 16 lanes of a row hit the same
 address), three register sets of 12 used in rotation, one group (10 steps at rate 5/6) ahead.
@@ -26,6 +26,10 @@ offset, v84 = LLR byte offset, v85 = minimum of the four metrics, v86 = LLR byte
 iteration: the refill then re-reads valid addresses).
 """
 import os
+import sys
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+from gen_lean_asm import coeffs                    # noqa: E402
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 OUT = os.environ.get("C8P_GEN_OUT4") or os.path.join(ROOT, "gr-ieee80211_amd", "csrc", "c8p_lean4_asm.h")
@@ -93,9 +97,8 @@ def gen_rate(cr):
         g = max(k for k in range(G) if gstart[k] <= i)
         return SET[g % 3] + (i - gstart[g])
 
-    def lpair(i):
-        r = lreg(i)
-        return "v[%d:%d]" % (r & ~1, (r & ~1) + 1), r & 1
+    def llr(i):
+        return "v%d" % lreg(i)
 
     L = []
     emit = L.append
@@ -139,29 +142,31 @@ def gen_rate(cr):
         dl = [delta(q, r) for r in range(4)]
         # ---- candidates
         if i0 is not None and i1 is not None:
-            p0, s0 = lpair(i0)
-            p1, s1 = lpair(i1)
             tabs = {}
             for kind in sorted(set(0 if d in (0, 3) else 1 for d in dl)):
                 t = TAB[len(tabs)]
                 tabs[kind] = t
                 # kind 0: {ka t0 + kb t1, sa t0 + sb t1};  kind 1: the t1 coefficients swapped {ka t0 + sb t1, sa t0 + kb t1}
                 sb = 1 if kind == 1 else 0
-                emit("v_pk_mul_f32 v[%d:%d], %%[kb%d], %s op_sel:[%d,%d] op_sel_hi:[%d,%d]" % (t, t + 1, q, p1, sb, s1, 1 - sb, s1))
-                emit("v_pk_fma_f32 v[%d:%d], %%[ka%d], %s, v[%d:%d] op_sel:[0,%d,0] op_sel_hi:[1,%d,1]" % (t, t + 1, q, p0, t, t + 1, s0, s0))
+                for h in (0, 1):
+                    emit("v_mul_f32_e32 v%d, %s, %%[%sb%d]" % (t + h, llr(i1), "ks"[h ^ sb], q))
+                for h in (0, 1):
+                    emit("v_fmac_f32_e32 v%d, %s, %%[%sa%d]" % (t + h, llr(i0), "ks"[h], q))
             for r in range(4):
                 d = dl[r]
                 t = tabs[0 if d in (0, 3) else 1]
                 sw = 1 if d in (3, 2) else 0      # delta 3: both coefficients swapped; delta 2 (t0 only) = kind 1 swapped
-                emit("v_pk_add_f32 v[%d:%d], v[%d:%d], v[%d:%d] op_sel:[0,%d] op_sel_hi:[0,%d]" % (C[r], C[r] + 1, M[r], M[r] + 1, t, t + 1, sw, 1 - sw))
+                for h in (0, 1):
+                    emit("v_add_f32_e32 v%d, v%d, v%d" % (C[r] + h, M[r], t + (h ^ sw)))
         else:
             for r in range(4):
                 d = dl[r]
                 if i0 is not None:
-                    p, s, sw, kk = lpair(i0) + ((d >> 1) & 1, "ka")
+                    sw, k, i = (d >> 1) & 1, "a", i0
                 else:
-                    p, s, sw, kk = lpair(i1) + (d & 1, "kb")
-                emit("v_pk_fma_f32 v[%d:%d], %%[%s%d], %s, v[%d:%d] op_sel:[%d,%d,0] op_sel_hi:[%d,%d,0]" % (C[r], C[r] + 1, kk, q, p, M[r], M[r] + 1, sw, s, 1 - sw, s))
+                    sw, k, i = d & 1, "b", i1
+                for h in (0, 1):
+                    emit("v_fma_f32 v%d, %%[%s%s%d], %s, v%d" % (C[r] + h, "ks"[h ^ sw], k, q, llr(i), M[r]))
         # ---- exchange, decision, record
         acc = lambda r: "v_addc_co_u32_e32 v%d, vcc, v%d, v%d, vcc" % (M[r] + 1, M[r] + 1, M[r] + 1)
         if q in DPP:
@@ -233,7 +238,7 @@ def gen_rate(cr):
     emit("s_mov_b32 %%[nblk], %s" % cnt)
     body = "\n".join('      "%s\\n\\t"' % x for x in L)
     clob = ['"vcc"', '"scc"', '"memory"'] + ['"s%d"' % (PTR + i) for i in range(8)] + ['"v%d"' % r for r in range(20, 87)]
-    ins = ['[ka%d] "v"(K[%d].a)' % (q, q) for q in range(6)] + ['[kb%d] "v"(K[%d].b)' % (q, q) for q in range(6)] + \
+    ins = coeffs() + \
           ['[initx] "v"(initx)', '[inity] "v"(inity)', '[flip] "v"(flip)', '[bound] "v"(bound)', '[segn] "s"(segn)', '[llr] "s"(llr)', '[sv] "s"(sv)']
     n_slots = sum(1 for x in L[L.index("1:"):L.index("s_sub_u32 %s, %s, 1" % (cnt, cnt))] if x.startswith("v_"))
     return """

@@ -7,15 +7,15 @@ block of the float step, same feed; k_rx_1ss_lds uses them).
   lean_blocks_int<CR>   the production fast path.  When every path metric of a block is known to stay POSITIVE, the unsigned
                         order of the float bit patterns is the float order, and the compare can be an integer subtract with
                         borrow.  That buys what the float domain cannot: a per-lane carry-IN, i.e. a per-lane tie rule, in the
-                        same instruction that reads the partner lane through DPP.  A DPP step is then 4 VALU instructions
-                        (candidates, borrow, record, max) instead of 5 (candidates, difference, class test, record, max).
+                        same instruction that reads the partner lane through DPP.  A DPP step is then 5 VALU instructions
+                        (two candidates, borrow, record, max) instead of 6 (two candidates, difference, class test, record, max).
   lean_blocks_asm<CR>   the float step of c8p_viterbi_lean.h, instruction for instruction (-DC8P_LEAN_ASM, experiments only).
 
 Why one asm statement: the borrow chain lives in VCC across every step of the loop, and the compiler may use VCC between two
 asm statements; DPP operands inside inline asm are also invisible to its hazard recogniser.
 
 The step (both flavours share the candidates):
-    cand  = {keep, send} = P + A(q) * t0 (+ B(q) * t1)          v_pk_fma_f32 (+ v_pk_mul_f32, v_pk_add_f32 when both LLRs exist)
+    cand  = {keep, send} = P + A(q) * t0 (+ B(q) * t1)          two v_fma_f32; when both LLRs exist two each of v_mul, v_fmac, v_add
   float:
     q <= 3:  d = recv - keep, pre = max(recv, keep)              v_sub_f32_dpp / v_max_f32_dpp   (q == 2: one v_mov_b32_dpp more)
     q >= 4:  swap, pre = max(a0, a1)                             v_permlane{16,32}_swap_b32, v_max_f32
@@ -37,8 +37,10 @@ The step (both flavours share the candidates):
       Before every block all lanes are checked against `bound` (c8p_viterbi_lean.h); the loop leaves at the first block whose
       start metrics do not guarantee positive candidates, and the caller runs that block with the float step.
 
-Registers: v62 = pre (read as the pair v[62:63] with both halves taken from v62), v63 = acc, v[56:57] / v[58:59] = candidate
-pairs (alternating), v[54:55] / v[60:61] = branch-metric pairs, v52 / v53 = d (alternating; integer: v52 = unused difference),
+Every float operation is a plain 32-bit one: packed FP32 (one instruction on a register pair) is not used anywhere in this engine.
+
+Registers: v62 = pre, v63 = acc, v56, v57 / v58, v59 = {keep, send} candidates (alternating), v54, v55 / v60, v61 = {keep, send}
+branch metrics, v52 / v53 = d (alternating; integer: v52 = unused difference),
 v51 = q=2 intermediate, v50 = byte offset of this lane's survivor dword.  SGPRs: two sets of LLR registers filled alternately
 (one load group in flight at a time), s[56:57] next block's LLRs, s[58:59] this block's, s60 blocks left, s[62:63] check mask.
 """
@@ -81,6 +83,11 @@ RM = " row_mask:0xf bank_mask:0xf"
 ADDC = "v_addc_co_u32_e32 v63, vcc, v63, v63, vcc"
 
 
+def coeffs():
+    """asm inputs: the lane's keep / send coefficients of t0 (ka, sa) and of t1 (kb, sb) in the six phases, one register each"""
+    return ['[%s%s%d] "v"(K[%d].%s.%s)' % (h, k, q, q, k, "xy"["ks".index(h)]) for k in "ab" for q in range(6) for h in "ks"]
+
+
 def gen_rate(cr, integer):
     n, G = NLB[cr], NGRP[cr]
     steps = [idx(cr, j) for j in range(BLK)]
@@ -98,9 +105,8 @@ def gen_rate(cr, integer):
         g = max(k for k in range(G) if gstart[k] <= i)
         return SETBASE[g % 2] + (i - gstart[g])
 
-    def sgpr_pair(i):
-        r = sreg(i)
-        return "s[%d:%d]" % (r & ~1, (r & ~1) + 1), r & 1
+    def llr(i):
+        return "s%d" % sreg(i)
 
     L = []
     emit = L.append
@@ -143,10 +149,9 @@ def gen_rate(cr, integer):
 
     def emit_tab(j):
         q, (i0, i1), t = j % 6, steps[j], tabreg[j]
-        p0, s0 = sgpr_pair(i0)
-        p1, s1 = sgpr_pair(i1)
-        emit("v_pk_mul_f32 v[%d:%d], %%[kb%d], %s op_sel:[0,%d] op_sel_hi:[1,%d]" % (t, t + 1, q, p1, s1, s1))
-        emit("v_pk_fma_f32 v[%d:%d], %%[ka%d], %s, v[%d:%d] op_sel:[0,%d,0] op_sel_hi:[1,%d,1]" % (t, t + 1, q, p0, t, t + 1, s0, s0))
+        for op, k, i in (("mul", "b", i1), ("fmac", "a", i0)):
+            for h in (0, 1):
+                emit("v_%s_f32_e32 v%d, %s, %%[%s%s%d]" % (op, t + h, llr(i), "ks"[h], k, q))
 
     def emit_pend(p):
         if p is None:
@@ -188,18 +193,17 @@ def gen_rate(cr, integer):
             if j not in hoisted:
                 emit_tab(j)
             t = tabreg[j]
-            emit("v_pk_add_f32 v[%d:%d], v[62:63], v[%d:%d] op_sel:[0,0] op_sel_hi:[0,1]" % (c, c + 1, t, t + 1))
+            for h in (0, 1):
+                emit("v_add_f32_e32 v%d, v62, v%d" % (c + h, t + h))
             # the next two-LLR step's pair, if its LLRs are already here (same load group): issued now, used ~5 steps later
             nx = [k for k in two if k > j]
             if nx and group_of_step(nx[0]) == group_of_step(j):
                 emit_tab(nx[0])
                 hoisted.add(nx[0])
-        elif i0 is not None:
-            p0, s0 = sgpr_pair(i0)
-            emit("v_pk_fma_f32 v[%d:%d], %%[ka%d], %s, v[62:63] op_sel:[0,%d,0] op_sel_hi:[1,%d,0]" % (c, c + 1, q, p0, s0, s0))
         else:
-            p1, s1 = sgpr_pair(i1)
-            emit("v_pk_fma_f32 v[%d:%d], %%[kb%d], %s, v[62:63] op_sel:[0,%d,0] op_sel_hi:[1,%d,0]" % (c, c + 1, q, p1, s1, s1))
+            k, i = ("a", i0) if i0 is not None else ("b", i1)
+            for h in (0, 1):
+                emit("v_fma_f32 v%d, %%[%s%s%d], %s, v62" % (c + h, "ks"[h], k, q, llr(i)))
         # the previous step's decision fills the two wait states the DPP / permlane read of the candidates needs
         emit_pend(pend)
         if q in DPP:
@@ -273,7 +277,7 @@ def gen_rate(cr, integer):
     body = "\n".join('      "%s\\n\\t"' % x for x in L)
     clob = ['"vcc"', '"scc"', '"memory"'] + ['"s%d"' % (PTR + i) for i in range(11)] + \
            ['"s%d"' % (b + i) for b in SETBASE for i in range(SETSZ)] + ['"v%d"' % r for r in range(50, 64)]
-    ins = ['[ka%d] "v"(K[%d].a)' % (q, q) for q in range(6)] + ['[kb%d] "v"(K[%d].b)' % (q, q) for q in range(6)]
+    ins = coeffs()
     if integer:
         ins += ['[init] "v"(init)', '[flip] "v"(flip)', '[bound] "s"(bound)', '[segn] "s"(segn)']
     else:
@@ -321,7 +325,7 @@ def gen_rate_lds(cr, integer=True):
     the 30 unrolled float steps wanted 10 more VGPRs than the rest of k_rx_1ss_lds)"""
     n = NLB[cr]
     GS, NS = LDS_GS[cr], LDS_NSETS[cr]
-    SW = 2 if GS == 2 else 4      # registers per set (even, so that every LLR sits in an even-aligned pair)
+    SW = 2 if GS == 2 else 4      # registers per set (even: a 64-bit LDS read writes an even-aligned pair)
     assert n % GS == 0
     G = n // GS
     assert G % NS == 0
@@ -335,9 +339,8 @@ def gen_rate_lds(cr, integer=True):
     def vreg(i):
         return VB + SW * (grp(i) % NS) + (i % GS)
 
-    def vpair(i):
-        r = vreg(i)
-        return "v[%d:%d]" % (r & ~1, (r & ~1) + 1), r & 1
+    def llr(i):
+        return "v%d" % vreg(i)
 
     def load_group(g, wrapped):
         """ds reads of group g of this block (wrapped: of the next block, whose LLRs follow at + 4 n bytes)"""
@@ -361,10 +364,9 @@ def gen_rate_lds(cr, integer=True):
 
     def emit_tab(j):
         q, (i0, i1), t = j % 6, steps[j], tabreg[j]
-        p0, s0 = vpair(i0)
-        p1, s1 = vpair(i1)
-        emit("v_pk_mul_f32 v[%d:%d], %%[kb%d], %s op_sel:[0,%d] op_sel_hi:[1,%d]" % (t, t + 1, q, p1, s1, s1), [grp(i1)])
-        emit("v_pk_fma_f32 v[%d:%d], %%[ka%d], %s, v[%d:%d] op_sel:[0,%d,0] op_sel_hi:[1,%d,1]" % (t, t + 1, q, p0, t, t + 1, s0, s0), [grp(i0)])
+        for op, k, i in (("mul", "b", i1), ("fmac", "a", i0)):
+            for h in (0, 1):
+                emit("v_%s_f32_e32 v%d, %s, %%[%s%s%d]" % (op, t + h, llr(i), "ks"[h], k, q), [grp(i)])
 
     def emit_pend(p):
         if p is None:
@@ -393,18 +395,17 @@ def gen_rate_lds(cr, integer=True):
             if j not in hoisted:
                 emit_tab(j)
             t = tabreg[j]
-            emit("v_pk_add_f32 v[%d:%d], v[62:63], v[%d:%d] op_sel:[0,0] op_sel_hi:[0,1]" % (c, c + 1, t, t + 1))
+            for h in (0, 1):
+                emit("v_add_f32_e32 v%d, v62, v%d" % (c + h, t + h))
             # the next two-LLR step's pair ahead of time (off the pre -> pre chain), if its LLRs are at most one group further on
             nx = [k for k in two if k > j]
             if nx and grp(steps[nx[0]][1]) <= grp(i1) + 1:
                 emit_tab(nx[0])
                 hoisted.add(nx[0])
-        elif i0 is not None:
-            p0, s0 = vpair(i0)
-            emit("v_pk_fma_f32 v[%d:%d], %%[ka%d], %s, v[62:63] op_sel:[0,%d,0] op_sel_hi:[1,%d,0]" % (c, c + 1, q, p0, s0, s0), [grp(i0)])
         else:
-            p1, s1 = vpair(i1)
-            emit("v_pk_fma_f32 v[%d:%d], %%[kb%d], %s, v[62:63] op_sel:[0,%d,0] op_sel_hi:[1,%d,0]" % (c, c + 1, q, p1, s1, s1), [grp(i1)])
+            k, i = ("a", i0) if i0 is not None else ("b", i1)
+            for h in (0, 1):
+                emit("v_fma_f32 v%d, %%[%s%s%d], %s, v62" % (c + h, "ks"[h], k, q, llr(i)), [grp(i)])
         emit_pend(pend)
         if q in DPP:
             if not integer:
@@ -471,7 +472,7 @@ def gen_rate_lds(cr, integer=True):
             L.append("s_waitcnt lgkmcnt(%d)" % next(wi) if it[0] == "wait" else it[1])
         text = "\n".join('      "%s\\n\\t"' % x for x in L)
         clob = ['"vcc"', '"memory"'] + ['"v%d"' % r for r in range(VA, 62) if r != 50]
-        ins = ['[ka%d] "v"(K[%d].a)' % (q, q) for q in range(6)] + ['[kb%d] "v"(K[%d].b)' % (q, q) for q in range(6)]
+        ins = coeffs()
         ins += ['[cls%d] "v"(K[%d].cls)' % (q, q) for q in range(4)] + ['[llr] "s"(llr)']
         n_valu = sum(1 for (x, rd) in body if x.startswith("v_"))
         return """
@@ -543,7 +544,7 @@ template <> __device__ __forceinline__ void lean_block_flt_lds<%d>(float& pre, u
     text = "\n".join('      "%s\\n\\t"' % x for x in L)
     fixed = (50, 62, 63)
     clob = ['"vcc"', '"scc"', '"memory"'] + ['"s%d"' % (PTR + i) for i in range(0, 11)] + ['"v%d"' % r for r in range(VA, 64) if r not in fixed]
-    ins = ['[ka%d] "v"(K[%d].a)' % (q, q) for q in range(6)] + ['[kb%d] "v"(K[%d].b)' % (q, q) for q in range(6)]
+    ins = coeffs()
     ins += ['[init] "v"(init)', '[flip] "v"(flip)', '[bound] "s"(bound)', '[segn] "s"(segn)', '[llr] "s"(llr)', '[sv] "s"(sv)']
     return """
 // code rate %s, LLRs from LDS: %d per block in %d groups of %d, %d register sets (v%d..v49), address in v%d; %d VALU instructions per 30 steps

@@ -23,17 +23,16 @@ g = lambda k: rows[k]["cyc_W8"]
 # the opcodes of the lean Viterbi step (csrc/c8p_viterbi_lean.h), priced at saturation (8 waves / SIMD)
 table = {
     "source": src,
-    "note": "cycles per wave64 instruction per SIMD, 8 waves / SIMD, independent chains; every VALU opcode of the step costs one "
-            "~4.15-cycle issue slot (packed f32, DPP, VOPC, carry ops, any SGPR operand), the permlane swaps two; only plain "
-            "VGPR-only v_add/sub/mul/mov/and/or/xor/lshrrev/fma issue at ~2.4 cycles, and only in dense runs (mixed into a "
-            "4-cycle stream they fill a whole slot: p_step_sign = p_step_cur)",
+    "note": "cycles per wave64 instruction per SIMD, 8 waves / SIMD, independent chains; DPP, VOPC, carry ops and anything with an SGPR "
+            "operand cost one ~4.15-cycle issue slot, the permlane swaps two; plain VGPR-only v_add/sub/mul/mov/and/or/xor/lshrrev/"
+            "fma/fmac issue at ~2.4 cycles, and only in dense runs (mixed into a 4-cycle stream they fill a whole slot)",
     "lean_step_opcodes": {
-        "v_pk_fma_f32": g("p_pk_fma_sgpr"), "v_pk_mul_f32": g("p_pk_mul"), "v_pk_add_f32": g("p_pk_add"),
+        "v_fma_f32": g("p_fma"), "v_mul_f32": g("p_mul"), "v_fmac_f32": g("p_fmac"), "v_add_f32": g("p_add"),
         "v_sub_f32_dpp": g("p_sub_dpp_quad"), "v_max_f32_dpp": g("p_max_dpp_quad"), "v_mov_b32_dpp": g("p_mov_dpp_quad"),
         "v_cmp_class_f32": g("p_cmpclass"), "v_cmp_gt_f32": g("p_cmpgt"), "v_addc_co_u32": g("p_addc"),
         "v_permlane16_swap_b32": g("p_swap16"), "v_permlane32_swap_b32": g("p_swap32"), "v_max_f32": g("p_max"),
         "v_or_b32": g("p_or"), "v_cmpx_class_f32": g("p_cmpclass"), "v_cmpx_gt_f32": g("p_cmpgt"),
-        # the integer-compare block loop (round 2 on): borrow / max through DPP, the swap phases' plain max / borrow, the carry shift's xor
+        # the integer-compare block loop: borrow / max through DPP, the swap phases' plain max / borrow, the carry shift's xor
         "v_subb_co_u32_dpp": g("p_subb_dpp"), "v_max_u32_dpp": g("p_max_u32_dpp"), "v_max_u32": g("p_max_u32"),
         "v_sub_co_u32": g("p_add_co"), "v_xor_b32": g("p_xor"),
     },

@@ -6,7 +6,7 @@
 // i.e. the SIMD's issue time per wave-instruction when W waves share it.  The same number from the wall clock
 // (event time x measured shader clock / instructions per SIMD) is printed beside it as a cross-check.
 //
-// build: hipcc --offload-arch=gfx950 -O3 -o tools/probe_issue.bin tools/probe_issue.hip ; run on the GPU box.
+// build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o tools/probe_issue.bin tools/probe_issue.hip ; run on the GPU box.
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cstdio>
@@ -26,8 +26,7 @@ struct Out { unsigned long long cyc, wall; };
   v2f p0 = {a0, a1}, p1 = {a2, a3}, p2 = {a4, a5}, p3 = {a6, a7}, q0 = {b0, b1}, q1 = {b2, b3};                       \
   unsigned u0 = threadIdx.x, u1 = 0x380;                                                                              \
   float s0 = seed[0], s1 = seed[1];                                                                                   \
-  v2f sp = {seed[2], seed[3]};                                                                                        \
-  (void)s0; (void)s1; (void)sp;                                                                                       \
+  (void)s0; (void)s1;                                                                                                 \
   __syncthreads();                                                                                                    \
   const unsigned long long t0 = clock64(), w0 = wall_clock64();
 
@@ -45,7 +44,7 @@ struct Out { unsigned long long cyc, wall; };
   [a0] "+v"(a0), [a1] "+v"(a1), [a2] "+v"(a2), [a3] "+v"(a3), [a4] "+v"(a4), [a5] "+v"(a5), [a6] "+v"(a6),           \
       [a7] "+v"(a7), [b0] "+v"(b0), [b1] "+v"(b1), [b2] "+v"(b2), [b3] "+v"(b3), [p0] "+v"(p0), [p1] "+v"(p1),       \
       [p2] "+v"(p2), [p3] "+v"(p3), [q0] "+v"(q0), [q1] "+v"(q1), [u0] "+v"(u0), [u1] "+v"(u1)
-#define INS [s0] "s"(s0), [s1] "s"(s1), [sp] "s"(sp)
+#define INS [s0] "s"(s0), [s1] "s"(s1)
 
 #define PROBE(NAME, BODY)                                                                                             \
   __global__ __launch_bounds__(1024) void NAME(float* sink, Out* out, const float* seed, int iters)                  \
@@ -67,7 +66,7 @@ struct Out { unsigned long long cyc, wall; };
 #define D8(OP, TAIL)                                                                                                  \
   OP " %[a0], %[a0]" TAIL "\n\t" OP " %[a0], %[a0]" TAIL "\n\t" OP " %[a0], %[a0]" TAIL "\n\t" OP " %[a0], %[a0]" TAIL "\n\t" \
   OP " %[a0], %[a0]" TAIL "\n\t" OP " %[a0], %[a0]" TAIL "\n\t" OP " %[a0], %[a0]" TAIL "\n\t" OP " %[a0], %[a0]" TAIL
-// packed: four chains x 2
+// 64-bit operands: four chains x 2
 #define P8(OP, TAIL)                                                                                                  \
   OP " %[p0], %[p0]" TAIL "\n\t" OP " %[p1], %[p1]" TAIL "\n\t" OP " %[p2], %[p2]" TAIL "\n\t" OP " %[p3], %[p3]" TAIL "\n\t" \
   OP " %[p0], %[p0]" TAIL "\n\t" OP " %[p1], %[p1]" TAIL "\n\t" OP " %[p2], %[p2]" TAIL "\n\t" OP " %[p3], %[p3]" TAIL
@@ -89,12 +88,6 @@ PROBE(p_mov, "v_mov_b32 %[a0], %[a1]\n\tv_mov_b32 %[a1], %[a2]\n\tv_mov_b32 %[a2
 PROBE(p_addu, "v_add_u32 %[a0], %[a0], %[u0]\n\tv_add_u32 %[a1], %[a1], %[u0]\n\tv_add_u32 %[a2], %[a2], %[u0]\n\tv_add_u32 %[a3], %[a3], %[u0]\n\t"
               "v_add_u32 %[a4], %[a4], %[u0]\n\tv_add_u32 %[a5], %[a5], %[u0]\n\tv_add_u32 %[a6], %[a6], %[u0]\n\tv_add_u32 %[a7], %[a7], %[u0]")
 PROBE(p_lshl_or, X8("v_lshl_or_b32", ", 1, %[u0]"))
-PROBE(p_pk_fma, P8("v_pk_fma_f32", ", %[q0], %[q1]"))
-PROBE(p_pk_fma_sgpr, P8("v_pk_fma_f32", ", %[sp], %[q1] op_sel_hi:[1,0,1]"))
-PROBE(p_pk_add, P8("v_pk_add_f32", ", %[q0]"))
-PROBE(p_pk_mul, P8("v_pk_mul_f32", ", %[q0]"))
-PROBE(p_pk_add_dep, "v_pk_add_f32 %[p0], %[p0], %[q0]\n\tv_pk_add_f32 %[p0], %[p0], %[q0]\n\tv_pk_add_f32 %[p0], %[p0], %[q0]\n\tv_pk_add_f32 %[p0], %[p0], %[q0]\n\t"
-                    "v_pk_add_f32 %[p0], %[p0], %[q0]\n\tv_pk_add_f32 %[p0], %[p0], %[q0]\n\tv_pk_add_f32 %[p0], %[p0], %[q0]\n\tv_pk_add_f32 %[p0], %[p0], %[q0]")
 // DPP as an operand modifier (sources are not written inside the body: no DPP read-after-VALU-write hazard)
 #define DPP8(OP, CTRL)                                                                                                \
   OP " %[a0], %[b0], %[b1]" CTRL "\n\t" OP " %[a1], %[b0], %[b1]" CTRL "\n\t" OP " %[a2], %[b1], %[b2]" CTRL "\n\t"   \
@@ -145,8 +138,8 @@ PROBE(p_swizzle, "ds_swizzle_b32 %[a0], %[a0] offset:0x401f\n\tds_swizzle_b32 %[
                  "ds_swizzle_b32 %[a4], %[a4] offset:0x401f\n\tds_swizzle_b32 %[a5], %[a5] offset:0x401f\n\tds_swizzle_b32 %[a6], %[a6] offset:0x401f\n\tds_swizzle_b32 %[a7], %[a7] offset:0x401f\n\ts_waitcnt lgkmcnt(0)")
 
 // ---- whole trellis steps, as the lean kernel issues them (dependent through a0 = path metric) ---------------------
-// (explicit registers v[100:107]: the packed result pair is read as two 32-bit DPP operands)
-// current q=0 step with one LLR: pk_fma(keep,send) ; [decision of the previous step] ; sub_dpp ; max_dpp       = 5 VALU
+// (explicit registers v100..v109)
+// current q=0 step with one LLR: 2 fma (keep, send) ; [decision of the previous step] ; sub_dpp ; max_dpp       = 6 VALU
 #define HARD "vcc", "s40", "s41", "v100", "v101", "v102", "v103", "v104", "v105", "v106", "v107", "v108", "v109"
 #define PROBE_HARD(NAME, BODY)                                                                                        \
   __global__ __launch_bounds__(1024) void NAME(float* sink, Out* out, const float* seed, int iters)                  \
@@ -163,16 +156,13 @@ PROBE(p_swizzle, "ds_swizzle_b32 %[a0], %[a0] offset:0x401f\n\tds_swizzle_b32 %[
     asm volatile("v_mov_b32 %0, v102" : "=v"(a0) :: HARD);                                                            \
     EPILOGUE                                                                                                          \
   }
-// v[102:103] = {pre, pre-copy}, v[106:107] = lane coefficients {ka, sa}, v[100:101] = {keep, send}, v104 = d
-PROBE_HARD(p_step_cur, "v_pk_fma_f32 v[100:101], v[106:107], %[sp], v[102:103] op_sel_hi:[1,0,0]\n\t"
+// v102 = pre, v106 / v107 = lane coefficients ka / sa, v100 / v101 = keep / send, v104 = d
+#define CAND "v_fma_f32 v100, v106, %[s0], v102\n\tv_fma_f32 v101, v107, %[s0], v102\n\t"
+PROBE_HARD(p_step_cur, CAND
                        "v_cmp_class_f32_e32 vcc, v104, %[u1]\n\tv_addc_co_u32_e32 %[u0], vcc, %[u0], %[u0], vcc\n\t"
                        "v_sub_f32_dpp v104, v101, v100" DPPQ "\n\tv_max_f32_dpp v102, v101, v100" DPPQ)
-// the same with two plain fmas instead of the packed one                                                       = 6 VALU
-PROBE_HARD(p_step_2fma, "v_fma_f32 v100, v106, %[s0], v102\n\tv_fma_f32 v101, v107, %[s0], v102\n\t"
-                        "v_cmp_class_f32_e32 vcc, v104, %[u1]\n\tv_addc_co_u32_e32 %[u0], vcc, %[u0], %[u0], vcc\n\t"
-                        "v_sub_f32_dpp v104, v101, v100" DPPQ "\n\tv_max_f32_dpp v102, v101, v100" DPPQ)
-// swap step (q = 4): pk_fma ; cmp ; addc ; swap ; max                                                          = 5 VALU
-PROBE_HARD(p_step_swap, "v_pk_fma_f32 v[100:101], v[106:107], %[sp], v[102:103] op_sel_hi:[1,0,0]\n\t"
+// swap step (q = 4): 2 fma ; cmp ; addc ; swap ; max                                                           = 6 VALU
+PROBE_HARD(p_step_swap, CAND
                         "v_cmp_gt_f32_e32 vcc, v104, v105\n\tv_addc_co_u32_e32 %[u0], vcc, %[u0], %[u0], vcc\n\t"
                         "v_permlane16_swap_b32 v100, v101\n\tv_max_f32 v102, v100, v101")
 // metric-only chain of the DPP step: fma, fma, (2 wait states filled by the hardware or not), max_dpp
@@ -230,42 +220,42 @@ PROBE(p_sub_dpp_b0, "v_sub_f32_dpp %[a0], %[b0], %[b1]" DPPQ "\n\tv_sub_f32 %[a1
 // LDS broadcast read (all lanes the same address): VALU-free delivery of uniform values into VGPRs
 PROBE(p_ldsbc_fma, "ds_read_b128 v[100:103], %[u1]\n\t" X8("v_fma_f32", ", %[b0], %[b1]") "\n\ts_waitcnt lgkmcnt(0)")
 // candidate new steps (explicit registers as above; v105 = sigma', v108 = acc)
-// DPP step with the sign trick: pk_fma ; sub_dpp ; max_dpp ; e = fma(sigma', d, +0) ; acc = alignbit(acc, e, 31)
-PROBE_HARD(p_step_sign, "v_pk_fma_f32 v[100:101], v[106:107], %[sp], v[102:103] op_sel_hi:[1,0,0]\n\t"
+// DPP step with the sign trick: 2 fma ; sub_dpp ; max_dpp ; e = fma(sigma', d, +0) ; acc = alignbit(acc, e, 31)
+PROBE_HARD(p_step_sign, CAND
                         "v_fma_f32 v105, v104, v106, 0\n\tv_alignbit_b32 %[u0], %[u0], v105, 31\n\t"
                         "v_sub_f32_dpp v104, v101, v100" DPPQ "\n\tv_max_f32_dpp v102, v101, v100" DPPQ)
-// swap step with the sign trick: pk_fma ; swap ; max ; e = a0 - a1 ; alignbit
-PROBE_HARD(p_step_swap_sign, "v_pk_fma_f32 v[100:101], v[106:107], %[sp], v[102:103] op_sel_hi:[1,0,0]\n\t"
+// swap step with the sign trick: 2 fma ; swap ; max ; e = a0 - a1 ; alignbit
+PROBE_HARD(p_step_swap_sign, CAND
                              "v_sub_f32 v105, v104, v103\n\tv_alignbit_b32 %[u0], %[u0], v105, 31\n\t"
                              "v_permlane16_swap_b32 v100, v101\n\tv_max_f32 v102, v100, v101")
 
 // ---- third set: integer-compare step (all candidates positive: unsigned order of the bit patterns = float order) and LDS-pipe
 // exchanges for the lane bits 4 / 5.  v108 = d (integer difference, unused), v109 = byte address of lane ^ 32 for ds_bpermute.
-// DPP step: pk_fma ; addc (records the previous decision, its carry-out = the per-lane tie rule of this step) ; subb_dpp ; max_u32_dpp
-PROBE_HARD(p_step_int, "v_pk_fma_f32 v[100:101], v[106:107], %[sp], v[102:103] op_sel_hi:[1,0,0]\n\t"
+// DPP step: 2 fma ; addc (records the previous decision, its carry-out = the per-lane tie rule of this step) ; subb_dpp ; max_u32_dpp
+PROBE_HARD(p_step_int, CAND
                        "v_addc_co_u32_e32 %[u0], vcc, %[u0], %[u0], vcc\n\ts_nop 0\n\t"
                        "v_subb_co_u32_dpp v108, vcc, v101, v100, vcc" DPPQ "\n\tv_max_u32_dpp v102, v101, v100" DPPQ)
 // the same with v_cndmask_b32_dpp as the selector
-PROBE_HARD(p_step_int_cnd, "v_pk_fma_f32 v[100:101], v[106:107], %[sp], v[102:103] op_sel_hi:[1,0,0]\n\t"
+PROBE_HARD(p_step_int_cnd, CAND
                            "v_addc_co_u32_e32 %[u0], vcc, %[u0], %[u0], vcc\n\ts_nop 0\n\t"
                            "v_subb_co_u32_dpp v108, vcc, v101, v100, vcc" DPPQ "\n\tv_cndmask_b32_dpp v102, v101, v100, vcc" DPPQ)
-// lane bit 4 through ds_swizzle (LDS pipe, no VALU slot), float compare: pk_fma ; swizzle ; cmp_class ; addc ; wait ; sub ; max
-PROBE_HARD(p_step_swz, "v_pk_fma_f32 v[100:101], v[106:107], %[sp], v[102:103] op_sel_hi:[1,0,0]\n\t"
+// lane bit 4 through ds_swizzle (LDS pipe, no VALU slot), float compare: 2 fma ; swizzle ; cmp_class ; addc ; wait ; sub ; max
+PROBE_HARD(p_step_swz, CAND
                        "v_cmp_class_f32_e32 vcc, v104, %[u1]\n\tds_swizzle_b32 v105, v101 offset:0x401f\n\t"
                        "v_addc_co_u32_e32 %[u0], vcc, %[u0], %[u0], vcc\n\ts_waitcnt lgkmcnt(0)\n\t"
                        "v_sub_f32 v104, v105, v100\n\tv_max_f32 v102, v105, v100")
-// lane bit 4 through ds_swizzle, integer compare: pk_fma ; swizzle ; addc ; wait ; subb ; max_u32
-PROBE_HARD(p_step_swz_int, "v_pk_fma_f32 v[100:101], v[106:107], %[sp], v[102:103] op_sel_hi:[1,0,0]\n\t"
+// lane bit 4 through ds_swizzle, integer compare: 2 fma ; swizzle ; addc ; wait ; subb ; max_u32
+PROBE_HARD(p_step_swz_int, CAND
                            "ds_swizzle_b32 v105, v101 offset:0x401f\n\t"
                            "v_addc_co_u32_e32 %[u0], vcc, %[u0], %[u0], vcc\n\ts_waitcnt lgkmcnt(0)\n\t"
                            "v_subb_co_u32_e32 v108, vcc, v105, v100, vcc\n\tv_max_u32 v102, v105, v100")
 // lane bit 5 through ds_bpermute, integer compare
-PROBE_HARD(p_step_bperm_int, "v_pk_fma_f32 v[100:101], v[106:107], %[sp], v[102:103] op_sel_hi:[1,0,0]\n\t"
+PROBE_HARD(p_step_bperm_int, CAND
                              "ds_bpermute_b32 v105, v109, v101\n\t"
                              "v_addc_co_u32_e32 %[u0], vcc, %[u0], %[u0], vcc\n\ts_waitcnt lgkmcnt(0)\n\t"
                              "v_subb_co_u32_e32 v108, vcc, v105, v100, vcc\n\tv_max_u32 v102, v105, v100")
-// swap step, integer compare: pk_fma ; swap ; addc ; sub_co ; max
-PROBE_HARD(p_step_swap_int, "v_pk_fma_f32 v[100:101], v[106:107], %[sp], v[102:103] op_sel_hi:[1,0,0]\n\t"
+// swap step, integer compare: 2 fma ; swap ; addc ; sub_co ; max
+PROBE_HARD(p_step_swap_int, CAND
                             "v_addc_co_u32_e32 %[u0], vcc, %[u0], %[u0], vcc\n\t"
                             "v_permlane16_swap_b32 v100, v101\n\tv_sub_co_u32_e32 v108, vcc, v100, v101\n\tv_max_u32 v102, v100, v101")
 PROBE(p_subb_dpp, "v_subb_co_u32_dpp %[a0], vcc, %[b0], %[b1], vcc" DPPQ "\n\tv_subb_co_u32_dpp %[a1], vcc, %[b1], %[b2], vcc" DPPQ "\n\t"
@@ -287,11 +277,6 @@ static const Probe probes[] = {
   E(p_mov, 8, "v_mov_b32"),
   E(p_addu, 8, "v_add_u32"),
   E(p_lshl_or, 8, "v_lshl_or_b32"),
-  E(p_pk_fma, 8, "v_pk_fma_f32 (VGPR operands)"),
-  E(p_pk_fma_sgpr, 8, "v_pk_fma_f32, SGPR pair operand + op_sel_hi (as in the lean step)"),
-  E(p_pk_add, 8, "v_pk_add_f32"),
-  E(p_pk_mul, 8, "v_pk_mul_f32"),
-  E(p_pk_add_dep, 8, "v_pk_add_f32 dependent"),
   E(p_sub_dpp_quad, 8, "v_sub_f32_dpp quad_perm:[1,0,3,2]"),
   E(p_max_dpp_quad, 8, "v_max_f32_dpp quad_perm:[1,0,3,2]"),
   E(p_max_dpp_ror8, 8, "v_max_f32_dpp row_ror:8"),
@@ -313,9 +298,8 @@ static const Probe probes[] = {
   E(p_smov_fma, 4, "s_mov_b32 ; v_fma_f32 (4 pairs, counted as 4)"),
   E(p_bpermute, 8, "ds_bpermute_b32 x8 + wait"),
   E(p_swizzle, 8, "ds_swizzle_b32 SWAP,16 x8 + wait"),
-  E(p_step_cur, 1, "lean step q=0, 1 LLR: pk_fma, cmp_class, addc, sub_dpp, max_dpp  (cycles per STEP)"),
-  E(p_step_2fma, 1, "same with two v_fma_f32 instead of v_pk_fma_f32             (cycles per STEP)"),
-  E(p_step_swap, 1, "lean step q=4: pk_fma, cmp_gt, addc, permlane16_swap, max       (cycles per STEP)"),
+  E(p_step_cur, 1, "lean step q=0, 1 LLR: 2 fma, cmp_class, addc, sub_dpp, max_dpp  (cycles per STEP)"),
+  E(p_step_swap, 1, "lean step q=4: 2 fma, cmp_gt, addc, permlane16_swap, max       (cycles per STEP)"),
   E(p_sub, 8, "v_sub_f32"), E(p_mul, 8, "v_mul_f32"), E(p_min, 8, "v_min_f32"),
   E(p_add_sgpr, 8, "v_add_f32 with an SGPR operand"),
   E(p_add_e64, 8, "v_add_f32_e64 (VOP3 encoding)"), E(p_add_neg, 8, "v_add_f32_e64 with a neg modifier"),
@@ -335,14 +319,14 @@ static const Probe probes[] = {
   E(p_add_sdwa, 8, "v_add_f32_sdwa (dword selects)"),
   E(p_sub_dpp_b0, 8, "v_sub_f32_dpp / v_sub_f32 alternating"),
   E(p_ldsbc_fma, 8, "8 v_fma_f32 + one broadcast ds_read_b128 (counted as 8)"),
-  E(p_step_sign, 1, "DPP step, sign trick: pk_fma, fma, alignbit, sub_dpp, max_dpp      (cycles per STEP)"),
-  E(p_step_swap_sign, 1, "swap step, sign trick: pk_fma, sub, alignbit, swap, max         (cycles per STEP)"),
-  E(p_step_int, 1, "DPP step, integer compare: pk_fma, addc, subb_dpp, max_u32_dpp            (cycles per STEP)"),
-  E(p_step_int_cnd, 1, "DPP step, integer compare: pk_fma, addc, subb_dpp, cndmask_dpp        (cycles per STEP)"),
-  E(p_step_swz, 1, "bit-4 step via ds_swizzle: pk_fma, swizzle, cmp_class, addc, sub, max      (cycles per STEP)"),
-  E(p_step_swz_int, 1, "bit-4 step via ds_swizzle, integer: pk_fma, swizzle, addc, subb, max_u32 (cycles per STEP)"),
-  E(p_step_bperm_int, 1, "bit-5 step via ds_bpermute, integer: pk_fma, bpermute, addc, subb, max_u32 (cycles per STEP)"),
-  E(p_step_swap_int, 1, "swap step, integer: pk_fma, addc, swap16, sub_co, max_u32              (cycles per STEP)"),
+  E(p_step_sign, 1, "DPP step, sign trick: 2 fma, fma, alignbit, sub_dpp, max_dpp      (cycles per STEP)"),
+  E(p_step_swap_sign, 1, "swap step, sign trick: 2 fma, sub, alignbit, swap, max         (cycles per STEP)"),
+  E(p_step_int, 1, "DPP step, integer compare: 2 fma, addc, subb_dpp, max_u32_dpp            (cycles per STEP)"),
+  E(p_step_int_cnd, 1, "DPP step, integer compare: 2 fma, addc, subb_dpp, cndmask_dpp        (cycles per STEP)"),
+  E(p_step_swz, 1, "bit-4 step via ds_swizzle: 2 fma, swizzle, cmp_class, addc, sub, max      (cycles per STEP)"),
+  E(p_step_swz_int, 1, "bit-4 step via ds_swizzle, integer: 2 fma, swizzle, addc, subb, max_u32 (cycles per STEP)"),
+  E(p_step_bperm_int, 1, "bit-5 step via ds_bpermute, integer: 2 fma, bpermute, addc, subb, max_u32 (cycles per STEP)"),
+  E(p_step_swap_int, 1, "swap step, integer: 2 fma, addc, swap16, sub_co, max_u32              (cycles per STEP)"),
   E(p_subb_dpp, 8, "v_subb_co_u32_dpp (vcc in/out)"),
   E(p_max_u32_dpp, 8, "v_max_u32_dpp quad_perm"),
   E(p_chain_dpp, 1, "metric chain only: fma, fma, s_nop 1, max_dpp                    (cycles per STEP)"),

@@ -11,7 +11,7 @@ import tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 FLAGS = ("--offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fno-fast-math -fhip-fp32-correctly-rounded-divide-sqrt "
-         "-mllvm -disable-promote-alloca-to-lds=1").split()
+         "-mllvm -disable-promote-alloca-to-lds=1 -Xclang -target-feature -Xclang -packed-fp32-ops").split()
 
 
 def main():

@@ -1,6 +1,6 @@
 // tools/probes/probe_sync_cost.hip — what asking an IDLE stream costs the host: hipStreamSynchronize, hipStreamQuery, hipEventQuery / hipEventSynchronize on a
 // finished event, hipEventRecord, an empty kernel launch; and the same with a second thread launching kernels on another stream (the block chain's case)
-// hipcc -O2 --offload-arch=gfx950 -o /tmp/probe_sync_cost tools/probes/probe_sync_cost.hip -lpthread
+// hipcc -O2 --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -o /tmp/probe_sync_cost tools/probes/probe_sync_cost.hip -lpthread
 #include <hip/hip_runtime.h>
 #include <atomic>
 #include <chrono>

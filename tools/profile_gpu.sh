@@ -34,7 +34,7 @@ for c in FETCH_SIZE WRITE_SIZE "SQ_WAVES SQ_INSTS_VALU SQ_INSTS_SALU SQ_INSTS_LD
   rocprofv3 --kernel-trace --pmc $c -d $OUT/raw_pmc_$n -o pmc --output-format csv -- python $PWD/tools/exp_rawchain.py > $OUT/raw_pmc_$n.log 2>&1
 done
 # the issue cost of every opcode of the lean step on THIS box (tools/probe_issue.hip; ~40 s): what bench.py's roofline_valu prices with
-/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -o $OUT/probe_issue.bin tools/probe_issue.hip > $OUT/probe_issue_build.log 2>&1 && $OUT/probe_issue.bin > $OUT/probe_issue.txt 2>&1
+/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops -o $OUT/probe_issue.bin tools/probe_issue.hip > $OUT/probe_issue_build.log 2>&1 && $OUT/probe_issue.bin > $OUT/probe_issue.txt 2>&1
 # the headline as the bench runs it — three slots, launches of consecutive batches co-resident — as a kernel trace: summarize_prof.py
 # turns the k_rx_1ss_lds dispatches into "time during which at least one is resident, per step"
 rocprofv3 --kernel-trace -d $OUT/trace3 -o ${TAG}_slots3 --output-format csv -- $BENCH --no-frontend --no-stream --no-sensitivity --steps 60 --repeats 1 --min-timed-s 0 > $OUT/trace3.log 2>&1
