@@ -237,10 +237,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 4))) voi
       unsigned* sv = (unsigned*)(surv + lay[q].surv_off);
       const float bq = lean_bound(__uint_as_float(flags[2 * n + q]));
       switch (t0.cr) {
-        case C8P_CR_12: lean_blocks<C8P_CR_12, false>(S, K, init, flip, bq, L, tq.total, sv, done + 1, segn); break;
-        case C8P_CR_23: lean_blocks<C8P_CR_23, false>(S, K, init, flip, bq, L, tq.total, sv, done + 1, segn); break;
-        case C8P_CR_34: lean_blocks<C8P_CR_34, false>(S, K, init, flip, bq, L, tq.total, sv, done + 1, segn); break;
-        default:        lean_blocks<C8P_CR_56, false>(S, K, init, flip, bq, L, tq.total, sv, done + 1, segn); break;
+        case C8P_CR_12: lean_blocks<C8P_CR_12>(S, K, init, flip, bq, L, sv, done + 1, segn); break;
+        case C8P_CR_23: lean_blocks<C8P_CR_23>(S, K, init, flip, bq, L, sv, done + 1, segn); break;
+        case C8P_CR_34: lean_blocks<C8P_CR_34>(S, K, init, flip, bq, L, sv, done + 1, segn); break;
+        default:        lean_blocks<C8P_CR_56>(S, K, init, flip, bq, L, sv, done + 1, segn); break;
       }
       xch[pp][lane] = S.pre;
       if (pp == 3) segc = S.segc;

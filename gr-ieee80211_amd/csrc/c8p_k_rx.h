@@ -104,10 +104,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(6, 6))) voi
     lean_k_unpack(kbits, lane, K);
     const float bound = lean_bound(negb);
     switch (t.cr) {
-      case C8P_CR_12: lean_blocks<C8P_CR_12>(S, K, init, flip, bound, out, safe, sv, upto, segn); break;
-      case C8P_CR_23: lean_blocks<C8P_CR_23>(S, K, init, flip, bound, out, safe, sv, upto, segn); break;
-      case C8P_CR_34: lean_blocks<C8P_CR_34>(S, K, init, flip, bound, out, safe, sv, upto, segn); break;
-      default:        lean_blocks<C8P_CR_56>(S, K, init, flip, bound, out, safe, sv, upto, segn); break;
+      case C8P_CR_12: lean_blocks<C8P_CR_12>(S, K, init, flip, bound, out, sv, upto, segn); break;
+      case C8P_CR_23: lean_blocks<C8P_CR_23>(S, K, init, flip, bound, out, sv, upto, segn); break;
+      case C8P_CR_34: lean_blocks<C8P_CR_34>(S, K, init, flip, bound, out, sv, upto, segn); break;
+      default:        lean_blocks<C8P_CR_56>(S, K, init, flip, bound, out, sv, upto, segn); break;
     }
   }
   if (!ok) return;

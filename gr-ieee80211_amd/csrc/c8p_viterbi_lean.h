@@ -285,7 +285,7 @@ __device__ __forceinline__ float lean_bound(float negb)    // wave-uniform (SGPR
   return __uint_as_float((unsigned)__builtin_amdgcn_readfirstlane((int)__float_as_uint(fmaf(negb, 1.01f, 1e-30f))));
 }
 
-// full survivor blocks [S.done, upto) of a packet whose first `n_llr` LLRs (at least the ones those blocks consume) are at Lg
+// full survivor blocks [S.done, upto) of a packet whose LLRs (at least the ones those blocks consume) are at Lg
 // Traceback hints: k_finish walks segments of `segn` survivor blocks in parallel (segn = ceil(T / (30 C8P_TB_SEGS)), c8p_seg_blocks) and has to
 // assume the lane each segment ends in.  In the last block of every segment the forward pass sets bit 30 of the survivor dword
 // (C8P_SV_HINT; a block holds 30 decisions in bits 29..0) on the lane(s) that hold the largest path metric at the block's end.
@@ -302,11 +302,9 @@ __device__ __forceinline__ float lean_bound(float negb)    // wave-uniform (SGPR
 #endif
 __device__ __forceinline__ int c8p_seg_blocks(int Tn) { return (Tn + C8P_TB_SEGS * C8P_SV_BLK - 1) / (C8P_TB_SEGS * C8P_SV_BLK); }
 
-// TOUCH = false: no scalar-cache touches in the float step (k_viterbi_lean4 runs single blocks from inside two nested loops, where
-// the compiler cannot keep the loop-carried touch registers in SGPRs)
-template <int CR, bool TOUCH = true>
+template <int CR>
 __device__ __forceinline__ void lean_blocks(LeanState& S, const LeanK (&K)[6], unsigned init, unsigned flip, float bound,
-                                            const float* __restrict__ Lg, int n_llr, unsigned* __restrict__ sv, int upto, int segn)
+                                            const float* __restrict__ Lg, unsigned* __restrict__ sv, int upto, int segn)
 {
   int segc = __builtin_amdgcn_readfirstlane(S.segc);           // (a local copy: asm "+s" operand)
   constexpr int PER = RateInfo<CR>::PER, NL = RateInfo<CR>::NL, REP = C8P_SV_BLK / PER, NLB = NL * REP;   // NLB: LLRs per block
@@ -315,9 +313,6 @@ __device__ __forceinline__ void lean_blocks(LeanState& S, const LeanK (&K)[6], u
   float x[NL];
   upto = __builtin_amdgcn_readfirstlane(upto);
   int left = __builtin_amdgcn_readfirstlane(upto - S.done);   // (wave-uniform; an asm "+s" operand)
-  // touch registers: loop-carried ("+s") so that they can never share an SGPR with x[] — the touches are still in
-  // flight when the next block's real loads are issued, and scalar loads may return in any order
-  unsigned d0 = 0, d1 = 0, d2 = 0, d3 = 0, d4 = 0;
   while (left > 0) {
     // integer compare: as many blocks as keep every metric above the bound
 #if !(defined(C8P_EXPERIMENTS) && defined(C8P_EXP_NO_INT))
@@ -334,23 +329,6 @@ __device__ __forceinline__ void lean_blocks(LeanState& S, const LeanK (&K)[6], u
     for (int r = 0; r < REP; r++, lb += NL) {
 #pragma unroll
       for (int i = 0; i < NL; i++) { x[i] = L[lb + i]; }
-      if (TOUCH && r == 0) {
-        // Scalar loads return out of order, so the only usable wait is lgkmcnt(0): a real prefetch of the next block
-        // would be drained by the wait of this one.  Instead, right after that wait (the x[] inputs force it before
-        // this statement), touch the scalar-cache lines of the NEXT block with throw-away loads: they complete during
-        // the 30 steps below, and the next block's loads hit the scalar cache instead of stalling on L2 / HBM.
-        const int nb = lb + NLB;                    // first LLR of the next block
-        c4float* nx = L + (nb + NLB <= n_llr ? nb : lb);   // never touch past the LLRs that exist (no branch: a join
-                                                           // would make the compiler drain the touches right away)
-        if (NLB * 4 > 192)
-          asm volatile("s_load_dword %0, %5, 0x0\n\ts_load_dword %1, %5, 0x40\n\ts_load_dword %2, %5, 0x80\n\t"
-                       "s_load_dword %3, %5, 0xc0\n\ts_load_dword %4, %5, %8"
-                       : "+s"(d0), "+s"(d1), "+s"(d2), "+s"(d3), "+s"(d4) : "s"(nx), "s"(x[0]), "s"(x[NL - 1]), "n"(NLB * 4 - 4));
-        else
-          asm volatile("s_load_dword %0, %4, 0x0\n\ts_load_dword %1, %4, 0x40\n\ts_load_dword %2, %4, 0x80\n\t"
-                       "s_load_dword %3, %4, %7"
-                       : "+s"(d0), "+s"(d1), "+s"(d2), "+s"(d3) : "s"(nx), "s"(x[0]), "s"(x[NL - 1]), "n"(NLB * 4 - 4));
-      }
       if (r == 0) lean_steps<CR, 0, false, true>(S.pre, K, x, S.acc, S.pend, PER);
       else lean_steps<CR, 0, false, false>(S.pre, K, x, S.acc, S.pend, PER);
     }
@@ -364,7 +342,6 @@ __device__ __forceinline__ void lean_blocks(LeanState& S, const LeanK (&K)[6], u
       segc = 0;
     }
     *(unsigned*)((char*)sv + S.voff) = word;
-    if (TOUCH) asm volatile("s_waitcnt lgkmcnt(0)" : "+s"(d0), "+s"(d1), "+s"(d2), "+s"(d3), "+s"(d4));   // touches land before the integer loop reuses SGPRs
     S.voff += 256u; left--; S.nflt++;
   }
   S.done = upto; S.segc = __builtin_amdgcn_readfirstlane(segc);   // (wave-uniform: keep it out of the VGPRs)
@@ -523,7 +500,7 @@ __device__ __forceinline__ void lean_forward(const float* __restrict__ Lg, int n
   lean_int_consts(lane, init, flip);
   LeanState S;
   lean_init(S, lane);
-  lean_blocks<CR>(S, K, init, flip, lean_bound(negb), Lg, n_llr, sv, Tn / C8P_SV_BLK, c8p_seg_blocks(Tn));
+  lean_blocks<CR>(S, K, init, flip, lean_bound(negb), Lg, sv, Tn / C8P_SV_BLK, c8p_seg_blocks(Tn));
   if (lane == 0) *n_float_blocks = (uint32_t)S.nflt;   // diagnostic (C8P_BUF_DECSTAT): blocks that did not qualify for the integer loop
   lean_tail<CR>(S, K, Lg, n_llr, Tn, sv);
 }

@@ -5,7 +5,10 @@ survivors, the one place that ever did, leave through coalesced vector stores.
 
 Packed FP32: no instruction that works on a register pair of floats, written by hand or formed by the compiler (some of their forms have
 given wrong results on this hardware, now and then and without an error): the text of the sources, every line that calls hipcc, and the
-assembly of the library's two builds (cross-compiled here with the Makefile's own command lines)."""
+assembly of the library's two builds (cross-compiled here with the Makefile's own command lines).
+
+Loads in inline asm: a statement waits for its own loads.  The compiler takes a statement's outputs as written when it ends, and gives
+their registers to other values: a load still in flight would then overwrite one of those, an address among them."""
 import os
 import re
 import shlex
@@ -108,3 +111,53 @@ def test_the_built_kernels_hold_no_packed_fp32_and_no_scalar_cache_write(assembl
         assert "k_rx_1ss_lds" in text and "v_fma_f32" in text, lib
         assert PACKED_FP32.search(text) is None, (lib, PACKED_FP32.search(text).group(0))
         assert SCALAR_CACHE_WRITE.search(text) is None, (lib, SCALAR_CACHE_WRITE.search(text).group(0))
+
+
+# an asm statement, or one of the probes' macros that make one of their text argument
+ASM = re.compile(r"\b(?:asm|__asm__)\b(?:\s+(?:volatile|__volatile__))?\s*\(|\bPROBE(?:_HARD)?\s*\(")
+LOAD = re.compile(r"\b(?:s_load|s_buffer_load|ds_read|ds_load|ds_bpermute|ds_permute|ds_swizzle|global_load|flat_load|buffer_load|scratch_load)\w*")
+LGKM0, VM0 = re.compile(r"s_waitcnt[^\n]*\blgkmcnt\(0\)"), re.compile(r"s_waitcnt[^\n]*\bvmcnt\(0\)")
+
+
+def asm_texts(src):
+    """the instruction text of every asm statement: its string literals up to the first ':' outside a literal"""
+    for m in ASM.finditer(src):
+        k, depth, text = m.end(), 1, []
+        while k < len(src) and depth:
+            if src[k] == '"':
+                lit = re.compile(r'"((?:[^"\\]|\\.)*)"', re.S).match(src, k)
+                text.append(lit.group(1))
+                k = lit.end()
+                continue
+            if src[k] == ":":
+                break
+            depth += {"(": 1, ")": -1}.get(src[k], 0)
+            k += 1
+        yield src.count("\n", 0, m.start()) + 1, "".join(text).replace("\\n", "\n").replace("\\t", " ")
+
+
+def unwaited(text):
+    """the last load of a statement that no full wait of its counter follows, or None (exact counts may stand between)"""
+    for kind, wait in ((r"^(?:s_|ds_)", LGKM0), (r"^(?!s_|ds_)", VM0)):
+        loads = [m for m in LOAD.finditer(text) if re.match(kind, m.group(0))]
+        if loads and not wait.search(text, loads[-1].end()):
+            return loads[-1].group(0)
+    return None
+
+
+def test_statement_reader():
+    t = dict(asm_texts('asm volatile("s_load_dword %0, %1, 0x0\\n\\t" "s_waitcnt lgkmcnt(0)" : "=s"(a) : "s"(p));\n asm("ds_read_b32 %0, %1" : "=v"(a) : "v"(p));'))
+    assert list(t) == [1, 2] and unwaited(t[1]) is None and unwaited(t[2]) == "ds_read_b32"
+    assert unwaited("global_load_dword v0, v1, s[0:1]\ns_waitcnt lgkmcnt(0)") == "global_load_dword"
+    assert unwaited("ds_read_b32 v0, v1\ns_waitcnt lgkmcnt(0)\nds_read_b32 v2, v1\ns_waitcnt lgkmcnt(1)") == "ds_read_b32"
+
+
+def test_asm_statements_wait_for_their_own_loads():
+    n, bad = 0, []
+    for p in source_files():
+        if p.endswith((".h", ".hip", ".cc", ".cpp", ".c")):
+            for line, text in asm_texts(open(p, errors="replace").read()):
+                n += bool(LOAD.search(text))
+                if unwaited(text):
+                    bad.append("%s:%d: %s" % (os.path.relpath(p, ROOT), line, unwaited(text)))
+    assert n >= 20 and bad == []                     # (the generated block loops and the probes' exchange bodies)
