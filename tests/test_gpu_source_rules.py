@@ -161,3 +161,45 @@ def test_asm_statements_wait_for_their_own_loads():
                 if unwaited(text):
                     bad.append("%s:%d: %s" % (os.path.relpath(p, ROOT), line, unwaited(text)))
     assert n >= 20 and bad == []                     # (the generated block loops and the probes' exchange bodies)
+
+
+REG = re.compile(r"\b([vs])(?:(\d+)\b|\[(\d+):(\d+)\])")
+
+
+def named_registers(text):
+    out = set()
+    for m in REG.finditer(re.sub(r"%\[\w+\]", "", text)):
+        lo, hi = (m.group(2), m.group(2)) if m.group(2) else (m.group(3), m.group(4))
+        out |= {m.group(1) + str(k) for k in range(int(lo), int(hi) + 1)}
+    return out
+
+
+def test_registers_an_asm_statement_names_are_declared():
+    """a register named in the text (not an operand) is bound to an operand or a clobber: the compiler counts the registers of a kernel,
+    and keeps live values out of them, by the declarations alone"""
+    csrc = os.path.join(ROOT, "gr-ieee80211_amd", "csrc")
+    n = 0
+    for f in sorted(os.listdir(csrc)):
+        if not f.endswith((".h", ".hip")):
+            continue
+        src = open(os.path.join(csrc, f)).read()
+        for line, text in asm_texts(src):
+            named = named_registers(text)
+            if named:
+                start = sum(len(x) + 1 for x in src.split("\n")[:line - 1])
+                decl = src[start:src.index(";\n", src.index(" : ", start))]
+                declared = set(re.findall(r'"([vs]\d+)"', decl)) | set(re.findall(r'\{([vs]\d+)\}', decl))
+                assert named <= declared, (f, line, sorted(named - declared))
+                n += 1
+    assert n >= 16
+    probe = open(os.path.join(ROOT, "tools", "probe_issue.hip")).read()
+    hard = set(re.findall(r'"([vs]\d+)"', re.search(r"#define HARD (.*)", probe).group(1)))
+    plain = set(re.findall(r'"([vs]\d+)"', re.search(r"asm volatile\(BODY : OPS : INS : (.*?)\)", probe).group(1)))
+    cand = re.search(r'#define CAND "(.*)"', probe).group(1)
+    assert named_registers(cand) <= hard
+    for m in re.finditer(r"^PROBE(_HARD)?\((\w+),", probe, re.M):
+        text = probe[m.end():probe.index("\nPROBE", m.end()) if "\nPROBE" in probe[m.end():] else probe.index("\nstruct Probe", m.end())]
+        text = re.sub(r"//.*", "", text)
+        text = re.sub(r"^#define (?:.*\\\n)*.*$", "", text, flags=re.M)
+        named = named_registers("".join(re.findall(r'"((?:[^"\\]|\\.)*)"', text, re.S)).replace("\\n", "\n").replace("\\t", " "))
+        assert named <= (hard if m.group(1) else plain), (m.group(2), sorted(named))

@@ -217,8 +217,6 @@ PROBE(p_mov_sgpr, "v_mov_b32 %[a0], %[s0]\n\tv_mov_b32 %[a1], %[s0]\n\tv_mov_b32
 PROBE(p_add_sdwa, X8("v_add_f32_sdwa", ", %[b0] dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:DWORD"))
 PROBE(p_sub_dpp_b0, "v_sub_f32_dpp %[a0], %[b0], %[b1]" DPPQ "\n\tv_sub_f32 %[a1], %[b0], %[b1]\n\tv_sub_f32_dpp %[a2], %[b1], %[b2]" DPPQ "\n\tv_sub_f32 %[a3], %[b0], %[b1]\n\t"
                     "v_sub_f32_dpp %[a4], %[b0], %[b3]" DPPQ "\n\tv_sub_f32 %[a5], %[b0], %[b1]\n\tv_sub_f32_dpp %[a6], %[b2], %[b1]" DPPQ "\n\tv_sub_f32 %[a7], %[b0], %[b1]")
-// LDS broadcast read (all lanes the same address): VALU-free delivery of uniform values into VGPRs
-PROBE(p_ldsbc_fma, "ds_read_b128 v[100:103], %[u1]\n\t" X8("v_fma_f32", ", %[b0], %[b1]") "\n\ts_waitcnt lgkmcnt(0)")
 // candidate new steps (explicit registers as above; v105 = sigma', v108 = acc)
 // DPP step with the sign trick: 2 fma ; sub_dpp ; max_dpp ; e = fma(sigma', d, +0) ; acc = alignbit(acc, e, 31)
 PROBE_HARD(p_step_sign, CAND
@@ -318,7 +316,6 @@ static const Probe probes[] = {
   E(p_writelane, 8, "v_writelane_b32"), E(p_mov_sgpr, 8, "v_mov_b32 from an SGPR"),
   E(p_add_sdwa, 8, "v_add_f32_sdwa (dword selects)"),
   E(p_sub_dpp_b0, 8, "v_sub_f32_dpp / v_sub_f32 alternating"),
-  E(p_ldsbc_fma, 8, "8 v_fma_f32 + one broadcast ds_read_b128 (counted as 8)"),
   E(p_step_sign, 1, "DPP step, sign trick: 2 fma, fma, alignbit, sub_dpp, max_dpp      (cycles per STEP)"),
   E(p_step_swap_sign, 1, "swap step, sign trick: 2 fma, sub, alignbit, swap, max         (cycles per STEP)"),
   E(p_step_int, 1, "DPP step, integer compare: 2 fma, addc, subb_dpp, max_u32_dpp            (cycles per STEP)"),
