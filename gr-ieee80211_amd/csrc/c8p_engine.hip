@@ -366,16 +366,9 @@ extern "C" c8p_ctx* c8p_create(const c8p_cfg* cfg)
     c->slots.resize(nslot);
     c->own_stream = cfg->stream == nullptr;
     for (int i = 0; i < nslot; i++) {
+      // (every stream of the engine at the default priority: work on streams of different priorities has hung the GPU)
       if (cfg->stream) c->slots[i].stream = (hipStream_t)cfg->stream;
-      else {
-        // C8P_STREAM_PRIORITY (read at create, like C8P_SLOTS): -1 = the device's highest priority — for the contexts whose small kernels
-        // sit in front of another context's long ones (detect / signal in front of rx on one GPU)
-        const char* pe = getenv("C8P_STREAM_PRIORITY");
-        int lo = 0, hi = 0;
-        (void)hipDeviceGetStreamPriorityRange(&lo, &hi);
-        const int pr = pe ? std::max(hi, std::min(lo, atoi(pe))) : 0;
-        if (hipStreamCreateWithPriority(&c->slots[i].stream, hipStreamNonBlocking, pr) != hipSuccess) { delete c; return nullptr; }
-      }
+      else if (hipStreamCreateWithFlags(&c->slots[i].stream, hipStreamNonBlocking) != hipSuccess) { delete c; return nullptr; }
     }
     c->s = &c->slots[0];
     c->cur = 0;

@@ -203,3 +203,23 @@ def test_registers_an_asm_statement_names_are_declared():
         text = re.sub(r"^#define (?:.*\\\n)*.*$", "", text, flags=re.M)
         named = named_registers("".join(re.findall(r'"((?:[^"\\]|\\.)*)"', text, re.S)).replace("\\n", "\n").replace("\\t", " "))
         assert named <= (hard if m.group(1) else plain), (m.group(2), sorted(named))
+
+
+PRIORITY = re.compile("StreamCreateWith" + "Priority|StreamPriority" + "Range|STREAM_" + r"PRIORITY|is_high_priority_" + r"stream\s*=\s*True|Stream\([^)]*\bpriority\s*=")
+
+
+def test_every_stream_has_the_default_priority():
+    """work on streams of different priorities has hung this hardware for good: no source asks for one, and no environment switch can"""
+    assert PRIORITY.search("torch.cuda.Stream(device=0, " + "priority=-1)") and not PRIORITY.search("torch.cuda.Stream(device=0)")
+    assert hits(PRIORITY) == []
+
+
+def test_the_library_cannot_make_a_stream_of_another_priority():
+    lib = os.path.join(ROOT, "gr-ieee80211_amd", "libc8p_rx.so")
+    if not os.path.exists(lib):
+        pytest.skip("libc8p_rx.so is not built")
+    import shutil
+    if shutil.which("nm") is None:
+        pytest.skip("no nm")
+    names = subprocess.run(["nm", "-D", "--undefined-only", lib], capture_output=True, text=True, check=True).stdout
+    assert "hipStreamCreateWithFlags" in names and PRIORITY.search(names) is None
