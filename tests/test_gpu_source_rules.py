@@ -210,7 +210,7 @@ PRIORITY = re.compile("StreamCreateWith" + "Priority|StreamPriority" + "Range|ST
 
 def test_every_stream_has_the_default_priority():
     """work on streams of different priorities has hung this hardware for good: no source asks for one, and no environment switch can"""
-    assert PRIORITY.search("torch.cuda.Stream(device=0, " + "priority=-1)") and not PRIORITY.search("torch.cuda.Stream(device=0)")
+    assert PRIORITY.search("torch.cuda.Stream" + "(device=0, priority=-1)") and not PRIORITY.search("torch.cuda.Stream(device=0)")
     assert hits(PRIORITY) == []
 
 
