@@ -442,7 +442,7 @@ __device__ __forceinline__ void lean_tail_l(LeanState& S, const LeanK (&K)[6], c
 // svSigDecoder::decode (cloud80211phy.cc:2001-2088) is the data decoder's recurrence at rate 1/2 over L = 24 (L-SIG), 48 (HT-SIG,
 // VHT-SIG-A) or 26 (VHT-SIG-B) steps, traced back from state 0.  The literal form (wave_sig_viterbi_exact: two ds_bpermute gathers, a
 // three-way select per candidate, two ballots per step) costs 31 VALU instructions per step and was 60 % of k_classify's instructions;
-// the lean step costs ~8 (lane = state under the rotating map, partner through DPP / permlane swap, decision into a per-lane shift
+// the lean step costs ~11 (lane = state under the rotating map, partner through DPP / permlane swap, decision into a per-lane shift
 // register) and is the same function for finite |LLR| <= 2^20 and L >= 6 (top of this file).  The LLRs are checked first; anything
 // else takes the literal form.  Decisions: step k in bit (29 - k) of accA for k < 30 when L > 30, else in bit (L - 1 - k) of acc.
 // Traceback on the scalar unit: the lane index D at time u + 1 spells input bit u in its bit (u mod 6) (state bit k lives in lane bit

@@ -522,7 +522,7 @@ def valu_roofline(kern_x, n_pkt, float_frac, profile_tag, T=11960):
     launch duration of this run.  Pricing at the nominal 2.4 GHz makes the fraction a lower bound (the shader clock under this
     load is 2.2-2.35 GHz).  One batch alone gives every SIMD 4 decoder waves; the arbiter serves the oldest wave first, so they
     finish one after the other and the last runs alone, latency-bound (profiles/r2b/decoder_wave_cycles.txt: 27 SIMD cycles per
-    wave-step at 4 waves, 24 at 8 waves, against 21.7 from the opcode costs) — the exclusive launch cannot reach the ceiling, the
+    wave-step at 4 waves, 24 at 8 waves, against 21.7 from the opcode costs, there with packed candidates) — the exclusive launch cannot reach the ceiling, the
     pipelined step (other batches fill the tail) is what `value` measures."""
     pdir = os.path.join(ROOT, "profiles", profile_tag)
     f_cost, f_pmc = os.path.join(pdir, "opcode_costs.json"), os.path.join(pdir, "pmc_hbm.json")
@@ -541,7 +541,8 @@ def valu_roofline(kern_x, n_pkt, float_frac, profile_tag, T=11960):
             other, other_src = max(0.0, k["sq_insts_valu"] * n_pkt / 4096.0 - dec_instr), os.path.relpath(f_pmc, ROOT)
             if k.get("valu_busy"):
                 busy = {"valu_busy": k["valu_busy"], "sq_active_inst_valu_quad_cycles": k.get("sq_active_inst_valu"), "grbm_gui_active_cycles_8xcd": k.get("grbm_gui_active"),
-                        "formula": "SQ_ACTIVE_INST_VALU x 4 / 1024 SIMDs / (GRBM_GUI_ACTIVE / 8 XCDs), averages per launch of the PMC passes (C8P_SLOTS=1)",
+                        "formula": "SQ_ACTIVE_INST_VALU x 4 / 1024 SIMDs / (GRBM_GUI_ACTIVE / 8 XCDs), averages per launch of the PMC passes (C8P_SLOTS=1); "
+                                   "every instruction counts four cycles, plain VGPR-only ones can issue in about two: the quotient may pass 1",
                         "source": os.path.relpath(f_pmc, ROOT) + " (= " + os.path.relpath(os.path.join(pdir, "pmc_summary.txt"), ROOT) + ")"}
     cycles += other * 4.15
     n_simd, clk = 256 * 4, 2.4e9

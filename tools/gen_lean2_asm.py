@@ -5,8 +5,8 @@ pass for TWO packets per wave, LLRs from LDS (lean2_lds<CR>), one inline-asm sta
 Layout.  A packet owns 32 lanes (two DPP rows) and two registers per lane: index D = l + 32 r (l = lane & 31, r = register) plays the
 role the lane index plays in c8p_viterbi_lean.h — state bit k lives in bit (k + t) mod 6 of D at time t.  Exchange phases q = 0..3
 cross a lane bit inside a DPP row, q = 4 crosses the row bit (v_permlane16_swap, which swaps rows 0 <-> 1 and 2 <-> 3, i.e. serves
-both packets at once), q = 5 crosses the REGISTER bit: both candidates are already in the lane, four plain VALU instructions per
-register pair instead of the six issue slots of the permlane32 swap step of the one-packet layout.  The branch-metric pair of a
+both packets at once), q = 5 crosses the REGISTER bit: both candidates are already in the lane, five plain VALU instructions per
+register pair instead of the seven issue slots of the permlane32 swap step of the one-packet layout.  The branch-metric pair of a
 step with both LLRs is computed once per wave-step and shared by the two registers (tools/gen_lean4_asm.py has the same idea with
 16 lanes x 4 registers; this is the half-way layout that still gives a 4096-packet batch two waves per SIMD).
 

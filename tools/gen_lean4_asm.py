@@ -5,8 +5,8 @@ pass for FOUR packets per wave (lean4_int<CR>), one inline-asm statement per cod
 Layout.  A packet owns one row of 16 lanes and four registers per lane: index D = l + 16 r (l = lane & 15, r = register) plays the
 role the lane index plays in c8p_viterbi_lean.h — state bit k lives in bit (k + t) mod 6 of D at time t.  Exchange phases q = 0..3
 cross a lane bit (DPP inside the row, as before); q = 4, 5 cross a REGISTER bit: both candidates are already in this lane, the step
-is four plain VALU instructions (candidates, max, borrow, record) instead of the six issue slots of a permlane swap step.  Per
-30 steps at rate 5/6: 128 issue slots per packet instead of 157 (tools/gen_lean_asm.py), because in addition the branch-metric pair of
+is five plain VALU instructions (two candidates, max, borrow, record) instead of the seven issue slots of a permlane swap step.  Per
+30 steps at rate 5/6: 165 VALU instructions per packet instead of 189 (tools/gen_lean_asm.py), because in addition the branch-metric pair of
 a step with both LLRs is computed once per wave-step and shared by the four registers.
 
 What differs per register is a compile-time fact: the class of a transition is GF(2)-linear in D, so register r sees class c XOR

@@ -25,9 +25,11 @@ table = {
     "source": src,
     "note": "cycles per wave64 instruction per SIMD, 8 waves / SIMD, independent chains; DPP, VOPC, carry ops and anything with an SGPR "
             "operand cost one ~4.15-cycle issue slot, the permlane swaps two; plain VGPR-only v_add/sub/mul/mov/and/or/xor/lshrrev/"
-            "fma/fmac issue at ~2.4 cycles, and only in dense runs (mixed into a 4-cycle stream they fill a whole slot)",
+            "fma issue at 2.2-2.4 cycles in dense runs, fma at 3.7 where every operand differs from the last instruction's",
     "lean_step_opcodes": {
-        "v_fma_f32": g("p_fma"), "v_mul_f32": g("p_mul"), "v_fmac_f32": g("p_fmac"), "v_add_f32": g("p_add"),
+        # the candidates, VGPR operands only, issued in keep / send pairs that share two of their operands: the least that such an
+        # instruction was seen to cost (p_fma, eight chains with operands of their own: 3.7), so that the sum stays a lower bound
+        "v_fma_f32": g("p_fma_dep"), "v_mul_f32": g("p_mul"), "v_fmac_f32": g("p_fma_dep"), "v_add_f32": g("p_add"),
         "v_sub_f32_dpp": g("p_sub_dpp_quad"), "v_max_f32_dpp": g("p_max_dpp_quad"), "v_mov_b32_dpp": g("p_mov_dpp_quad"),
         "v_cmp_class_f32": g("p_cmpclass"), "v_cmp_gt_f32": g("p_cmpgt"), "v_addc_co_u32": g("p_addc"),
         "v_permlane16_swap_b32": g("p_swap16"), "v_permlane32_swap_b32": g("p_swap32"), "v_max_f32": g("p_max"),
